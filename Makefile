@@ -1,6 +1,7 @@
 # Builds the MI355X-native hot path (libtsdf_hip.so, gfx950 only) and the CPU oracle.
 # hipcc cross-compiles for gfx950 without a GPU present.
-ROOT    := $(dir $(abspath $(lastword $(MAKEFILE_LIST))))
+THIS    := $(abspath $(lastword $(MAKEFILE_LIST)))
+ROOT    := $(dir $(THIS))
 HIPCC   ?= /opt/rocm/bin/hipcc
 ARCH    ?= gfx950
 CSRC    := $(ROOT)tracking_sdf_amd/csrc
@@ -9,8 +10,12 @@ LIB     := $(LIBDIR)/libtsdf_hip.so
 
 # -ffp-contract=off and no fast-math are REQUIRED for parity: every multiply-add of the reference is
 # two roundings (its g++ build sets no -O/-march flags, src/CMakeLists.txt:97-98).
+# Packed FP32 (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32) stays switched off for EVERY piece of device code, probes included:
+# hipcc makes it from ordinary float code, and some of its forms have given wrong results on these machines now and then.
+# (The host pass does not know the feature and says so: harmless.)
+NO_PACKED_FP32 := -Xclang -target-feature -Xclang -packed-fp32-ops
 HIPEXTRA ?=
-HIPFLAGS := $(HIPEXTRA) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math \
+HIPFLAGS := $(HIPEXTRA) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -ffp-contract=off -fno-fast-math $(NO_PACKED_FP32) \
             -fhip-fp32-correctly-rounded-divide-sqrt -fno-slp-vectorize -Wall -Wextra -Wno-unused-parameter
 KERNELS := $(CSRC)/integrate_kernels.hip $(CSRC)/track_kernels.hip $(CSRC)/volume_kernels.hip $(CSRC)/preproc_kernels.hip $(CSRC)/mesh_kernels.hip
 HOSTSRC := $(CSRC)/api_core.cpp $(CSRC)/api_frames.cpp $(CSRC)/api_hotpath.cpp $(CSRC)/api_comm.cpp $(CSRC)/api_volume.cpp \
@@ -30,11 +35,11 @@ IDFLAG := -DTSDF_BUILD_ID='"$(BUILD_ID)"'
 all: lib oracle
 lib: $(LIB) $(HSACO)
 
-$(LIB): $(SRCS) $(HDRS)
+$(LIB): $(SRCS) $(HDRS) $(THIS)
 	@mkdir -p $(LIBDIR)
 	$(HIPCC) $(HIPFLAGS) $(IDFLAG) -shared -o $@ -x hip $(SRCS) -ldl -pthread -lhsa-runtime64
 
-$(HSACO): $(TRACK_DEPS)
+$(HSACO): $(TRACK_DEPS) $(THIS)
 	@mkdir -p $(LIBDIR)
 	$(HIPCC) $(HIPFLAGS) $(IDFLAG) --genco --no-gpu-bundle-output -o $@ -x hip $(CSRC)/track_kernels.hip
 
@@ -67,13 +72,13 @@ sdf_offline: $(LIB)
 # measured HBM ceiling for the roofline (streaming RMW over volume-shaped arrays); run on the GPU box
 rmw_probe:
 	@mkdir -p $(ROOT)build
-	$(HIPCC) --offload-arch=gfx950 -O3 -o $(ROOT)build/rmw_probe $(ROOT)tools/rmw_probe.hip
+	$(HIPCC) --offload-arch=gfx950 $(NO_PACKED_FP32) -O3 -o $(ROOT)build/rmw_probe $(ROOT)tools/rmw_probe.hip
 .PHONY: rmw_probe
 
 # known-byte kernels for calibrating rocprofv3's FETCH_SIZE / WRITE_SIZE (tools/pmc_calibrate.py); run on the GPU box
 pmc_calibrate:
 	@mkdir -p $(ROOT)build
-	$(HIPCC) --offload-arch=gfx950 -O3 -o $(ROOT)build/pmc_calibrate $(ROOT)tools/pmc_calibrate.hip
+	$(HIPCC) --offload-arch=gfx950 $(NO_PACKED_FP32) -O3 -o $(ROOT)build/pmc_calibrate $(ROOT)tools/pmc_calibrate.hip
 .PHONY: pmc_calibrate
 
 # the reference's exact call signatures (hotpath.hpp -DTSDF_WITH_EIGEN_PCL -DTSDF_WITH_ROS) against the mock Eigen /
@@ -103,6 +108,6 @@ shim_fields_demo: $(LIB)
 # (tools/aql_probe.hip); run on the GPU box: build/aql_probe build/aql_probe_kernel.hsaco
 aql_probe:
 	@mkdir -p $(ROOT)build
-	$(HIPCC) --offload-arch=gfx950 -O2 --genco --no-gpu-bundle-output -DPROBE_DEVICE_ONLY -o $(ROOT)build/aql_probe_kernel.hsaco $(ROOT)tools/aql_probe.hip
-	$(HIPCC) --offload-arch=gfx950 -O2 -o $(ROOT)build/aql_probe $(ROOT)tools/aql_probe.hip -lhsa-runtime64
+	$(HIPCC) --offload-arch=gfx950 $(NO_PACKED_FP32) -O2 --genco --no-gpu-bundle-output -DPROBE_DEVICE_ONLY -o $(ROOT)build/aql_probe_kernel.hsaco $(ROOT)tools/aql_probe.hip
+	$(HIPCC) --offload-arch=gfx950 $(NO_PACKED_FP32) -O2 -o $(ROOT)build/aql_probe $(ROOT)tools/aql_probe.hip -lhsa-runtime64
 .PHONY: aql_probe

@@ -10,8 +10,8 @@
 //         rings the doorbell -- no runtime call on the path
 // and reports, per submission: host time inside the submission, and the round trip submission -> word seen by the host.
 // Build (make aql_probe):
-//   hipcc --offload-arch=gfx950 -O2 --genco --no-gpu-bundle-output -o build/aql_probe_kernel.hsaco tools/aql_probe.hip -DPROBE_DEVICE_ONLY
-//   hipcc --offload-arch=gfx950 -O2 -o build/aql_probe tools/aql_probe.hip -lhsa-runtime64
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 --genco --no-gpu-bundle-output -o build/aql_probe_kernel.hsaco tools/aql_probe.hip -DPROBE_DEVICE_ONLY
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o build/aql_probe tools/aql_probe.hip -lhsa-runtime64
 #include <hip/hip_runtime.h>
 
 // the kernel: no blockDim / gridDim (code-object-v5 kernels read those from hidden arguments the probe does not fill)

@@ -2,7 +2,7 @@
 // A 640x480 frame is 8.3 MB as planes (xyz | nrm | rgb), 1.5 MB as raw depth + rgb.  For page-locked source buffers of these
 // sizes: the time of ONE hipMemcpyAsync + wait (latency form) and of 20 copies queued back to back on a stream (throughput
 // form), alone and next to a kernel that keeps the chip's memory system busy (a float4 read-modify-write sweep over 2 GiB).
-// Build: hipcc --offload-arch=gfx950 -O2 -o build/h2d_probe tools/h2d_probe.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o build/h2d_probe tools/h2d_probe.hip
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <cstdio>

@@ -2,7 +2,7 @@
 //   paths (1.3 KB of arguments): the <<<>>> syntax (hipLaunchKernel with an argument-pointer array, what the library
 //   uses), hipModuleLaunchKernel with the arguments pre-marshalled in one buffer, hipExtLaunchKernel;
 //   sizes: <<<>>> with 64 B .. 3840 B of arguments.
-// Build: hipcc --offload-arch=gfx950 -O2 -o build/launch_probe tools/launch_probe.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o build/launch_probe tools/launch_probe.hip
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <cstdio>

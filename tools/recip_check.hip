@@ -1,6 +1,6 @@
 // recip_check.hip -- exhaustive check of recip_ieee_small (tsdf_kernels.hip) against the compiler's IEEE division:
 // every float in [1e-5f, 4.0f].  Build + run on the GPU box:
-//   hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -o build/recip_check tools/recip_check.hip && build/recip_check
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -o build/recip_check tools/recip_check.hip && build/recip_check
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstring>

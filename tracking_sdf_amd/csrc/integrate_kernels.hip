@@ -375,15 +375,14 @@ __device__ __forceinline__ double exp_taylor8(double x) {
 //     lands within 2 units of an integer (about once in 10^4 wavefronts);
 //   * volume reads and stores are raw buffer operations on a 512-byte / 1-KiB descriptor of the item's segment:
 //     dead lanes carry an out-of-range offset and touch no memory -- no branch, no EXEC juggling, exact s_waitcnt counts;
-//   * the four f32 divisions of the running averages (one for D, three for the colour) run two at a time as packed
-//     f32 operations with the division's own FMA sequence (exactly the instruction sequence hipcc emits for
-//     a correctly rounded `/`, minus the range scaling, which a guard proves unnecessary or else takes the `/` path);
+//   * the four f32 divisions of the running averages (one for D, three for the colour, which share one reciprocal) run
+//     the division's own FMA sequence (exactly the instruction sequence hipcc emits for a correctly rounded `/`, minus
+//     the range scaling, which a guard proves unnecessary or else takes the `/` path);
 //   * the pre-rounded (float)cosine of the colour weight rides in the pixel record (weight-1 voxels use it as it is);
 //     a wavefront with lanes in the exp() band recomputes the f64 cosine from the record's normal for those lanes
 //     (a per-pixel plane of f64 cosines gathered per item was measured twice and lost both times: one more
 //     vector-memory instruction per item).
 
-typedef float v2f __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x3 __attribute__((ext_vector_type(3)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -542,27 +541,25 @@ __device__ __forceinline__ void project_item(const ProjConst& c, const ItemDesc&
     pixb = __umul24(iu1, c.su) + __umul24(iw1, c.sv);
 }
 
-// Correctly rounded n / b for two quotients at a time: hipcc's own sequence for `/` (v_rcp_f32, two Newton FMAs,
-// quotient, two residual corrections) WITHOUT its v_div_scale / v_div_fixup wrappers.  The wrappers only act when b,
-// 1/b, n/b or a residual leaves the normal range; callers check the operands (div_guard) and use `/` otherwise.
-__device__ __forceinline__ v2f rcp_refined(v2f b) {
-    v2f r = v2f{__builtin_amdgcn_rcpf(b.x), __builtin_amdgcn_rcpf(b.y)};
-    return __builtin_elementwise_fma(__builtin_elementwise_fma(-b, r, v2f{1.0f, 1.0f}), r, r);
+// Correctly rounded n / b: hipcc's own sequence for `/` (v_rcp_f32, two Newton FMAs, quotient, two residual corrections)
+// WITHOUT its v_div_scale / v_div_fixup wrappers.  The wrappers only act when b, 1/b, n/b or a residual leaves the normal
+// range; callers check the operands (tiny_lanes, kBits2p64) and use `/` otherwise.  One quotient per instruction: the
+// build keeps packed FP32 switched off (Makefile).
+__device__ __forceinline__ float rcp_refined(float b) {
+    const float r = __builtin_amdgcn_rcpf(b);
+    return __builtin_fmaf(__builtin_fmaf(-b, r, 1.0f), r, r);
 }
-__device__ __forceinline__ v2f div_core(v2f n, v2f b, v2f r) {
-    v2f q = n * r;
-    q = __builtin_elementwise_fma(__builtin_elementwise_fma(-b, q, n), r, q);
-    q = __builtin_elementwise_fma(__builtin_elementwise_fma(-b, q, n), r, q);
+__device__ __forceinline__ float div_core(float n, float b, float r) {
+    float q = n * r;
+    q = __builtin_fmaf(__builtin_fmaf(-b, q, n), r, q);
+    q = __builtin_fmaf(__builtin_fmaf(-b, q, n), r, q);
     return q;
 }
 // Range guard of the division core.  Numerators: n * 2^-26 is subnormal exactly for 0 < |n| < 2^-100 (zero stays zero).
 // State words (W, Color_W) as integers: 0 <= x < 2^64 <=> bits(x) < bits(2^64) (negative, inf, NaN are larger); the
 // new weight added to them lies in [0, 1], so b = state + weight stays within [0, 2^64] -- and b = 0 means n = 0 too
 // (both products vanish), which the core turns into the same NaN as 0/0.
-__device__ __forceinline__ unsigned long long tiny_lanes(v2f n) {
-    const v2f t = n * v2f{0x1p-26f, 0x1p-26f};
-    return lanes_subnormal(t.x) | lanes_subnormal(t.y);
-}
+__device__ __forceinline__ unsigned long long tiny_lanes(float n) { return lanes_subnormal(n * 0x1p-26f); }
 constexpr unsigned kBits2p64 = 0x5f800000u;
 
 struct GatherState {        // stage 1 done: pixel record requested
@@ -880,43 +877,43 @@ __global__ __launch_bounds__(kIntegrateBlock, kIntegrateMinWaves) void integrate
         const unsigned n_live = (unsigned)__popcll(uin.live);
         n_own += owned3 ? n_live : 0u;
         n_halo += owned3 ? 0u : n_live;
-        // sdf.cpp:289-292 (D, W) and :294-304 (colour), as packed f32 pairs {D-average, R} and {G, B}.  One item in eight
+        // sdf.cpp:289-292 (D, W) and :294-304 (colour), one reciprocal for D and one for the colour.  One item in eight
         // updates nothing (r04_integrate_fixed_costs.json): its averages are skipped -- the stores below stay where they are
         // (every lane's offset is out of range), so the count of vector-memory operations per step does not change.
-        v2f sum1 = v2f{0.f, 0.f}, q1 = v2f{0.f, 0.f}, q2 = v2f{0.f, 0.f};
+        float sum_w = 0.f, sum_c = 0.f, avg_d = 0.f, avg_r = 0.f, avg_g = 0.f, avg_b = 0.f;
         if (uin.live != 0ull) {
             const float W = __uint_as_float(uin.old.y), D = __uint_as_float(uin.old.x);
-            const float cx = __uint_as_float(uin.col.x);
-            const float wc = COLOR ? uin.wc : 0.f;
-            v2f num1, num2 = v2f{0.f, 0.f};
-            sum1.x = W + uin.w_new;
-            num1.x = W * D + uin.w_new * uin.d_new;
+            sum_w = W + uin.w_new;
+            const float num_d = W * D + uin.w_new * uin.d_new;
+            avg_d = div_core(num_d, sum_w, rcp_refined(sum_w));
+            unsigned long long bad = tiny_lanes(num_d) | lanes(uin.old.y >= kBits2p64);
+            float num_r = 0.f, num_g = 0.f, num_b = 0.f;
             if (COLOR) {
+                const float cx = __uint_as_float(uin.col.x), wc = uin.wc;
                 const unsigned rgb = uin.rgb;
                 const float pr = (float)(rgb & 255u), pg = (float)((rgb >> 8) & 255u), pb = (float)((rgb >> 16) & 255u);
-                sum1.y = cx + wc;
-                num1.y = cx * __uint_as_float(uin.col.y) + wc * pr;
-                num2 = v2f{cx, cx} * v2f{__uint_as_float(uin.col.z), __uint_as_float(uin.col.w)} + v2f{wc, wc} * v2f{pg, pb};
-            } else {
-                sum1.y = 1.0f; num1.y = 0.0f;
+                sum_c = cx + wc;
+                num_r = cx * __uint_as_float(uin.col.y) + wc * pr;
+                num_g = cx * __uint_as_float(uin.col.z) + wc * pg;
+                num_b = cx * __uint_as_float(uin.col.w) + wc * pb;
+                const float rc = rcp_refined(sum_c);
+                avg_r = div_core(num_r, sum_c, rc);
+                avg_g = div_core(num_g, sum_c, rc);
+                avg_b = div_core(num_b, sum_c, rc);
+                bad |= tiny_lanes(num_r) | tiny_lanes(num_g) | tiny_lanes(num_b) | lanes(uin.col.x >= kBits2p64);
             }
-            const v2f r = rcp_refined(sum1);
-            q1 = div_core(num1, sum1, r);
-            if (COLOR) q2 = div_core(num2, v2f{sum1.y, sum1.y}, v2f{r.y, r.y});
-            unsigned long long bad = tiny_lanes(num1) | lanes(uin.old.y >= kBits2p64);
-            if (COLOR) bad |= tiny_lanes(num2) | lanes(uin.col.x >= kBits2p64);
             if (__builtin_expect((bad & uin.live) != 0ull, 0)) {
-                q1.x = num1.x / sum1.x;
-                if (COLOR) { q1.y = num1.y / sum1.y; q2.x = num2.x / sum1.y; q2.y = num2.y / sum1.y; }
+                avg_d = num_d / sum_w;
+                if (COLOR) { avg_r = num_r / sum_c; avg_g = num_g / sum_c; avg_b = num_b / sum_c; }
             }
         }
         const __amdgpu_buffer_rsrc_t seg_dw = __builtin_amdgcn_make_buffer_rsrc(dw + base3, 0, 64 * (int)sizeof(float2), kRsrcWord3);
-        u32x2 o2; o2.x = __float_as_uint(q1.x); o2.y = __float_as_uint(sum1.x);
+        u32x2 o2; o2.x = __float_as_uint(avg_d); o2.y = __float_as_uint(sum_w);
         unsigned off8 = uin.off8;
         __builtin_amdgcn_raw_buffer_store_b64(o2, seg_dw, (int)off8, 0, 0);
         if (COLOR) {
             const __amdgpu_buffer_rsrc_t seg_c = __builtin_amdgcn_make_buffer_rsrc(crgb + base3, 0, 64 * (int)sizeof(float4), kRsrcWord3);
-            u32x4 c4; c4.x = __float_as_uint(sum1.y); c4.y = __float_as_uint(q1.y); c4.z = __float_as_uint(q2.x); c4.w = __float_as_uint(q2.y);
+            u32x4 c4; c4.x = __float_as_uint(sum_c); c4.y = __float_as_uint(avg_r); c4.z = __float_as_uint(avg_g); c4.w = __float_as_uint(avg_b);
             __builtin_amdgcn_raw_buffer_store_b128(c4, seg_c, (int)(off8 << 1), 0, 2);   // dropped stays out of range; nt: colour is streamed
         }
 
