@@ -1,6 +1,8 @@
 // aql_queue.cpp -- see aql_queue.hpp.  Host code only (HSA runtime API); gfx950 / code object v5.
 #include "aql_queue.hpp"
 
+#include "host_util.hpp"
+
 #include <hip/hip_runtime_api.h>
 #include <hsa/hsa.h>
 #include <hsa/hsa_ext_amd.h>
@@ -107,6 +109,15 @@ bool AqlQueue::init(int hip_device, const char* hsaco_path, const char* symbol_p
         std::fclose(f);
         if (!ok) { if (err) *err = std::string("cannot read ") + hsaco_path; destroy(); return false; }
     }
+    // The code object must be THIS build's: it carries the hash of the tracker's sources and flags in a constant.  Read from
+    // the image, before anything of it is loaded: a copy back from the loaded constant would have the runtime page-lock this
+    // function's stack, and page-locking memory that already exists is refused on these machines (the queue was then never used).
+    std::string id;
+    if (!build_id || !*build_id || !host::elf_string_constant(image.data(), image.size(), "tsdf_track_build_id", &id) || id != build_id) {
+        if (err) *err = std::string("the code object ") + hsaco_path + " is not this library's build (id '" + id + "', wanted '" + (build_id ? build_id : "") + "')";
+        destroy();
+        return false;
+    }
     hsa_code_object_reader_t reader;
     st = hsa_code_object_reader_create_from_memory(image.data(), image.size(), &reader);
     if (st != HSA_STATUS_SUCCESS) { set_err(err, "hsa_code_object_reader_create_from_memory", st); destroy(); return false; }
@@ -118,24 +129,6 @@ bool AqlQueue::init(int hip_device, const char* hsaco_path, const char* symbol_p
     st = hsa_executable_load_agent_code_object(exe, ap.gpu, reader, nullptr, nullptr);
     if (st == HSA_STATUS_SUCCESS) st = hsa_executable_freeze(exe, nullptr);
     if (st != HSA_STATUS_SUCCESS) { set_err(err, "loading the code object", st); destroy(); return false; }
-    // the code object must be THIS build's: it carries the hash of the tracker's sources and flags in a device variable
-    {
-        hsa_executable_symbol_t idsym;
-        uint64_t addr = 0;
-        uint32_t size = 0;
-        char got[64] = {0};
-        const size_t want_len = build_id ? std::strlen(build_id) : 0;
-        st = hsa_executable_get_symbol_by_name(exe, "tsdf_track_build_id", &ap.gpu, &idsym);
-        if (st == HSA_STATUS_SUCCESS) st = hsa_executable_symbol_get_info(idsym, HSA_EXECUTABLE_SYMBOL_INFO_VARIABLE_ADDRESS, &addr);
-        if (st == HSA_STATUS_SUCCESS) st = hsa_executable_symbol_get_info(idsym, HSA_EXECUTABLE_SYMBOL_INFO_VARIABLE_SIZE, &size);
-        if (st == HSA_STATUS_SUCCESS && addr && size > 0 && size < sizeof got) st = hsa_memory_copy(got, reinterpret_cast<const void*>(addr), size);
-        else if (st == HSA_STATUS_SUCCESS) st = HSA_STATUS_ERROR_INVALID_SYMBOL_NAME;
-        if (st != HSA_STATUS_SUCCESS || !want_len || std::strncmp(got, build_id, sizeof got) != 0) {
-            if (err) *err = std::string("the code object ") + hsaco_path + " is not this library's build (id '" + got + "', wanted '" + (build_id ? build_id : "") + "')";
-            destroy();
-            return false;
-        }
-    }
     SymbolPick sp{symbol_prefix, {}, false};
     st = hsa_executable_iterate_agent_symbols(exe, ap.gpu, pick_symbol, &sp);
     if (st != HSA_STATUS_SUCCESS || !sp.have) { if (err) *err = std::string("no kernel ") + symbol_prefix + "* in the code object"; destroy(); return false; }

@@ -1,6 +1,7 @@
 // host_util.cpp -- see host_util.hpp.  Host code only (no HIP): builds with plain g++ and under the sanitizers.
 #include "host_util.hpp"
 
+#include <elf.h>
 #include <fcntl.h>
 #include <sys/mman.h>
 #include <sys/stat.h>
@@ -182,6 +183,44 @@ int shm_fan_in(const ShmSegment& s, unsigned long long seq, int n, double* red, 
     }
     std::memcpy(red, sum, (size_t)n * sizeof(double));
     return TSDF_OK;
+}
+
+bool elf_string_constant(const char* image, size_t bytes, const char* symbol, std::string* text) {
+    if (!image || !symbol || !text) return false;
+    const auto inside = [bytes](uint64_t off, uint64_t len) { return off <= bytes && len <= bytes - off; };
+    const auto get = [&](uint64_t off, void* to, size_t len) {
+        if (!inside(off, len)) return false;
+        std::memcpy(to, image + off, len);       // nothing in an image read from a file is known to be aligned
+        return true;
+    };
+    Elf64_Ehdr eh;
+    if (!get(0, &eh, sizeof eh) || std::memcmp(eh.e_ident, ELFMAG, SELFMAG) != 0 || eh.e_ident[EI_CLASS] != ELFCLASS64 ||
+        eh.e_ident[EI_DATA] != ELFDATA2LSB || eh.e_shentsize != sizeof(Elf64_Shdr)) return false;
+    const auto section = [&](uint32_t n, Elf64_Shdr* sh) {
+        return n < eh.e_shnum && eh.e_shoff <= bytes && get(eh.e_shoff + (uint64_t)n * sizeof *sh, sh, sizeof *sh);
+    };
+    const size_t want = std::strlen(symbol) + 1;
+    for (uint32_t n = 0; n < eh.e_shnum; ++n) {
+        Elf64_Shdr tab, names, home;
+        if (!section(n, &tab)) return false;
+        if (tab.sh_type != SHT_DYNSYM && tab.sh_type != SHT_SYMTAB) continue;
+        if (!inside(tab.sh_offset, tab.sh_size) || !section(tab.sh_link, &names) || !inside(names.sh_offset, names.sh_size)) return false;
+        for (uint64_t at = 0; at + sizeof(Elf64_Sym) <= tab.sh_size; at += sizeof(Elf64_Sym)) {
+            Elf64_Sym sy;
+            if (!get(tab.sh_offset + at, &sy, sizeof sy)) return false;
+            if (sy.st_name > names.sh_size || want > names.sh_size - sy.st_name ||
+                std::memcmp(image + names.sh_offset + sy.st_name, symbol, want) != 0) continue;
+            if (!section(sy.st_shndx, &home) || home.sh_type == SHT_NOBITS || !inside(home.sh_offset, home.sh_size) ||
+                sy.st_value < home.sh_addr || sy.st_value - home.sh_addr > home.sh_size ||
+                sy.st_size > home.sh_size - (sy.st_value - home.sh_addr)) return false;
+            const char* at_text = image + home.sh_offset + (sy.st_value - home.sh_addr);
+            const void* end = std::memchr(at_text, 0, sy.st_size);
+            if (!end) return false;
+            text->assign(at_text, static_cast<const char*>(end));
+            return true;
+        }
+    }
+    return false;
 }
 
 }  // namespace host

@@ -263,5 +263,9 @@ void shm_publish(const ShmSegment& s, unsigned long long seq, const double* row 
 // wait for every rank's row of pass `seq`; sum the leading n entries in rank order into red (the others: this rank's own)
 int shm_fan_in(const ShmSegment& s, unsigned long long seq, int n, double* red /* kShmRowDoubles */, std::string* err);
 
+// The text a constant of an ELF64 image (a code object) starts with, read from the image itself: its NUL-terminated bytes,
+// no device and no loader involved.  False: not such an image, no such symbol, or anything that points outside the image.
+bool elf_string_constant(const char* image, size_t bytes, const char* symbol, std::string* text);
+
 }  // namespace host
 }  // namespace tsdf
