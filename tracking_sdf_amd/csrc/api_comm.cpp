@@ -34,7 +34,6 @@ void peer_close(tsdf_handle* h) {
 void shm_close(tsdf_handle* h) {
     if (!h->shm.active()) return;
     (void)hipStreamSynchronize(h->stream);
-    if (h->shm.dev_base) (void)hipHostUnregister(h->shm.base);
     shm_unmap(&h->shm);
 }
 
@@ -73,7 +72,8 @@ int tsdf_comm_init(tsdf_handle* h, int32_t nranks, int32_t rank, const void* id1
 }
 
 // The rendezvous on the named segment (host::shm_rendezvous, host_util.cpp: exclusive creation by rank 0, generation,
-// unlink once everybody has joined) needs no device; what is added here is the device alias of the mapping.
+// unlink once everybody has joined) needs no device, and the segment is touched by hosts only: it is never page-locked
+// for the device (memory that exists already cannot be on every machine, and the refusal's error would surface later).
 int tsdf_comm_init_shm(tsdf_handle* h, int32_t nranks, int32_t rank, const char* name) {
     int rc = check_ready(h, false);
     if (rc) return rc;
@@ -85,18 +85,6 @@ int tsdf_comm_init_shm(tsdf_handle* h, int32_t nranks, int32_t rank, const char*
         rc = shm_rendezvous(name, nranks, rank, &h->shm, &serr);
         if (rc) return fail(h, rc, "%s", serr.c_str());
     }
-    char* const base = h->shm.base;
-    const size_t bytes = h->shm.bytes;
-    // The device alias is only needed when a rank's final kernel writes its slot itself (host fold off); with the
-    // default host fold the segment is touched by hosts only, so a failed registration is not fatal.
-    hipError_t e = hipHostRegister(base, bytes, hipHostRegisterMapped | hipHostRegisterPortable);
-    void* dptr = nullptr;
-    if (e == hipSuccess) {
-        e = hipHostGetDevicePointer(&dptr, base, 0);
-        if (e != hipSuccess) { (void)hipHostUnregister(base); dptr = nullptr; }
-    }
-    if (e != hipSuccess) { (void)hipGetLastError(); dptr = nullptr; }
-    h->shm.dev_base = (char*)dptr;
     h->pass_seq = 0;               // every rank counts passes from the same origin
     return TSDF_OK;
 }

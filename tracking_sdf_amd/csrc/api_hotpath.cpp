@@ -60,19 +60,12 @@ int accumulate_pass(tsdf_handle* h, bool reduce_ranks, bool later_pass) {
     const bool use_peer = reduce_ranks && !use_rccl && h->peer.active();
     const bool use_shm = reduce_ranks && !use_rccl && !use_peer && h->shm.active();
     const unsigned long long seq = ++h->pass_seq;
-    // Where the last workgroup of track_kernel publishes this rank's finished row: pinned host memory (the host then
-    // also publishes it into the shared segment with a host store), or -- TSDF_HOST_FOLD=0 -- straight into this rank's
-    // slot of the shared segment through its device alias, tagged with the generation the other ranks wait for.
-    const bool dev_publish_shm = use_shm && !h->host_fold;
-    if (dev_publish_shm && !h->shm.dev_base)
-        return fail(h, TSDF_E_COMM, "shared-memory fan-in with device publishing needs the segment registered with HIP, which failed");
-    double* host_row = dev_publish_shm
-        ? reinterpret_cast<double*>(h->shm.dev_base + shm_slot_offset(h->shm, h->shm.rank, seq)) : h->red_host;
-    const unsigned long long dev_word = dev_publish_shm ? shm_word(h->shm, seq) : seq;
     if (h->timing_track) HIP_TRY(h, hipEventRecord(h->ev_track.a, h->stream));
-    // the row ends up on this host anyway (no in-stream all-reduce, no device-published slot): let the device stop
-    // after the shard level and add the <= 8 shard rows here
-    const bool host_fanin = !use_rccl && !use_peer && !dev_publish_shm && !h->timing_track;
+    // The row ends up on this host anyway (no in-stream all-reduce, no exchange on the device): let the device stop after
+    // the shard level and add the <= 8 shard rows here.  Otherwise -- and between ranks with TSDF_HOST_FOLD=0 -- the last
+    // workgroup of track_kernel finishes the row and leaves it in pinned host memory.  The shared segment of the ranks is
+    // written by the host in both cases.
+    const bool host_fanin = !use_rccl && !use_peer && !(use_shm && !h->host_fold) && !h->timing_track;
     // device-side exchange: the workgroup that finishes the row swaps it with the other ranks before handing it out
     PeerExchange px;
     if (use_peer) px = peer_exchange_for(h, seq);
@@ -82,7 +75,7 @@ int accumulate_pass(tsdf_handle* h, bool reduce_ranks, bool later_pass) {
     const bool via_aql = h->aql_on && h->aql.ready() && later_pass && host_fanin && !from_plane;
     bool took_queue = false;
     HIP_TRY(h, launch_track_folded(h->stream, p, h->dw, h->samples, h->partials, h->fold_ctr + (seq & 1ull) * track_fold_counter_words(), h->red_dev,
-                                   use_rccl ? nullptr : host_row, host_fanin ? h->shard_host : nullptr, dev_word, seq,
+                                   use_rccl ? nullptr : h->red_host, host_fanin ? h->shard_host : nullptr, seq, seq,
                                    use_peer ? &px : nullptr, via_aql ? &h->aql : nullptr, &took_queue));
     if (took_queue) h->cnt.track_passes_own_queue++;          // counted only when the queue really took the dispatch
     if (from_plane && h->deferred_list_samples) h->deferred.samples_listed = true;
@@ -150,11 +143,6 @@ int accumulate_pass(tsdf_handle* h, bool reduce_ranks, bool later_pass) {
         track_unpack_row(tot, h->red_host);
         if (stale) h->red_host[27] = std::nan("");
         arrived = true;
-    } else if (dev_publish_shm) {
-        std::string serr;
-        const int rc2 = shm_fan_in(h->shm, seq, kRedAllreduce, h->red_host, &serr);
-        if (rc2) return fail(h, rc2, "%s", serr.c_str());
-        arrived = true;
     } else {
         // The last workgroup (or the publish kernel) releases the pass number after the row (system scope); spinning on
         // it saves the runtime's completion-signal path.  Bounded: fall back to a real synchronisation.
@@ -167,7 +155,7 @@ int accumulate_pass(tsdf_handle* h, bool reduce_ranks, bool later_pass) {
         }
     }
     if (!arrived) HIP_TRY(h, hipStreamSynchronize(h->stream));
-    if (use_shm && !dev_publish_shm) {
+    if (use_shm) {
         // this rank's finished row is in red_host: publish it with a host store, then add everybody's rows
         shm_publish(h->shm, seq, h->red_host);
         std::string serr;

@@ -179,7 +179,7 @@ struct tsdf_handle {
     double* red_dev = nullptr;     // kRedWidth
     double* red_host = nullptr;    // pinned, kRedWidth doubles + the pass-number word the host polls
     unsigned long long pass_seq = 0;
-    bool host_fold = true;         // shared-memory fan-in: the host publishes this rank's row (TSDF_HOST_FOLD=0: the device writes the slot itself)
+    bool host_fold = true;         // shared-memory fan-in: the host adds this rank's shard rows (TSDF_HOST_FOLD=0: the device adds them)
     unsigned* fold_ctr = nullptr;  // arrival counters of the in-launch fan-in of track_kernel: two sets, alternating by pass parity
     // Gauss-Newton passes >= 1 of a tsdf_track call go through a user-mode queue of the library's own (2.3 us per pass less
     // than hipLaunchKernel: profiles/r05_aql_probe.json) when the row is handed to this host anyway (single rank / host

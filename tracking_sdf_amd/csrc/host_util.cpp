@@ -48,7 +48,7 @@ void shm_unmap(ShmSegment* s) {
     munmap(s->base, s->bytes);
     // the name was unlinked by rank 0 as soon as every rank had joined (shm_rendezvous): nothing to remove
     // here, and by now the name may belong to somebody else
-    s->base = s->dev_base = nullptr;
+    s->base = nullptr;
     s->nranks = 0;
 }
 
@@ -147,7 +147,7 @@ int shm_rendezvous(const char* name, int nranks, int rank, ShmSegment* out, std:
             base = nullptr;
         }
     }
-    out->nranks = nranks; out->rank = rank; out->base = base; out->dev_base = nullptr;
+    out->nranks = nranks; out->rank = rank; out->base = base;
     out->bytes = bytes; out->header = header; out->gen = gen; out->name = name;
     return TSDF_OK;
 }

@@ -237,7 +237,6 @@ inline volatile unsigned long long* shm_hdr(char* base, int word) {
 struct ShmSegment {
     int nranks = 0, rank = 0;
     char* base = nullptr;        // host mapping (header, then the slots)
-    char* dev_base = nullptr;    // device-visible alias (hipHostRegister; set by the caller)
     size_t bytes = 0, header = 0;
     unsigned long long gen = 0;  // generation of this segment (chosen by rank 0 at init), part of every published word
     std::string name;

@@ -268,7 +268,7 @@ struct TrackFold {               // in-launch fan-in of the per-workgroup rows
     unsigned* ctr;               // kTrackShards shard counters + 1 top counter, one 128-byte line each, zero between passes
     double* shard_rows;          // kTrackShards x kPartWidth
     double* red_dev;             // kRedWidth: result row for an in-stream all-reduce (may be null)
-    double* host_row;            // pinned host (or shared-segment alias): kRedWidth doubles + the word (may be null)
+    double* host_row;            // pinned host: kRedWidth doubles + the word (may be null)
     double* host_shards;         // pinned host, kTrackShards x kShardSlotDoubles: when given, the shard rows go to the host
                                  // (each behind its own word) and the second fan-in level runs there
     unsigned long long word;     // what is released behind host_row once it is complete
