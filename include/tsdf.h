@@ -390,7 +390,8 @@ int tsdf_comm_init_shm(tsdf_handle *h, int32_t nranks, int32_t rank, const char 
  * segment carries the IPC handles); TSDF_E_COMM when the runtime refuses IPC, and nothing is left configured then.
  * Two handles of ONE process (same pid and process token) lend each other their raw buffer pointers instead of IPC
  * mappings: such sibling handles must leave the exchange (tsdf_comm_finalize / tsdf_destroy) before any of them is
- * destroyed. */
+ * destroyed.  The exchange buffer (1 KiB per rank) is not given back before the process ends, so a process sets an
+ * exchange up a few times, not per frame. */
 int tsdf_comm_init_peer(tsdf_handle *h, int32_t nranks, int32_t rank, const char *name);
 int tsdf_comm_finalize(tsdf_handle *h);                          /* drop the RCCL communicator / the shared segment / the peer mappings (hook, if any, takes over) */
 /* Alternative: let the host do the 28-double sum (e.g. torch.distributed); fn = NULL removes it. */

@@ -7,7 +7,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "tracking_sdf_amd", "csrc")
-CASES = ["shm_registers_nothing"]
+CASES = ["shm_registers_nothing", "peer_keeps_its_buffer"]
 
 
 @pytest.fixture(scope="module")

@@ -27,7 +27,9 @@ void peer_close(tsdf_handle* h) {
     h->peer.mapped.clear();
     h->peer.via_ipc.clear();
     if (h->peer.bases_dev) (void)hipFree(h->peer.bases_dev);
-    if (h->peer.own) (void)hipFree(h->peer.own);
+    // The exchange buffer itself stays allocated until the process ends: uncached memory that a kernel has read is not given
+    // back (allocations made after such a free have held wrong values).  Nor is it used again: a rank that has not left the
+    // old exchange may still store into it.  1 KiB per rank of the exchange, once per set-up.
     h->peer.bases_dev = nullptr; h->peer.own = nullptr; h->peer.nranks = 0;
 }
 
