@@ -13,15 +13,18 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # file that names them keeps the whole tree from being run there.
 SCALAR_CACHE_WRITES = re.compile(r"\bs_(?:(?:buffer_|scratch_)?(?:store_(?:dword|b\d)|atomic_)|dcache_(?:wb|discard))", re.I)
 PROGRAM_TEXT = (".hip", ".cpp", ".hpp", ".c", ".h", ".s", ".py", ".sh", ".patch", ".diff", ".cmake", ".mk")
-NOT_SOURCE = {"build", "lib", "_work", "gpurun_out", "__pycache__"}      # built files and scratch folders, none of them tracked
+SOURCE_FOLDERS = ("include", "oracle", "profiles", "tests", "tools", "tracking_sdf_amd")
 
 
 def program_files():
-    for folder, subs, names in os.walk(ROOT):
-        subs[:] = sorted(s for s in subs if s not in NOT_SOURCE and not s.startswith("."))
-        for n in sorted(names):
-            if n.endswith(PROGRAM_TEXT) or n == "Makefile":
-                yield os.path.join(folder, n)
+    for n in sorted(os.listdir(ROOT)):
+        if os.path.isfile(os.path.join(ROOT, n)) and (n.endswith(PROGRAM_TEXT) or n == "Makefile"):
+            yield os.path.join(ROOT, n)
+    for top in SOURCE_FOLDERS:
+        for folder, _, names in os.walk(os.path.join(ROOT, top)):
+            for n in sorted(names):
+                if n.endswith(PROGRAM_TEXT) or n == "Makefile":
+                    yield os.path.join(folder, n)
 
 
 def test_the_pattern_knows_the_instructions():
